@@ -30,7 +30,13 @@ DEVINLINE float gate(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
 // Tiles of few rows: WM x WN waves, SLOTS whole tiles in LDS, each asked for SLOTS - 1 ahead.
 // Bound by the bytes of W.  Where one tile has all rows (ONCE), they are read past the caches (57344 x
-// 8192, 61 rows: 50 us kept in them, 46 so; 512 rows, where tiles share W: 37 kept, 42 not).
+// 8192, 61 rows: 50 us kept in them, 46 so; 512 rows, where tiles share W: 37 kept, 42 not).  There a
+// loop over all of K begins at another pair of tiles from column to column, as workgroups at the
+// same one ask for the same part of every row at a time (us, at the same | turned: 57344 x 8192,
+// 61 rows of 6 bits 52.9 | 47.3, 17 rows 50.0 | 48.5; 8 experts of 4096 x 14336, 50 rows of 6 bits
+// each 61.1 | 56.1; 4 of 8200 x 8192, 13 rows of 6 bits 46.2 | 42.2; 28672 x 4096, 64 rows 19.1 |
+// 19.5).  A part of K does not: parts are apart already (10240 x 8192 in two, 61 rows 22.7 | 23.5;
+// 8192 x 28672 in four 36.2 | 35.7).
 //
 // Scales are what costs most to load: a row's are in a line of their own, and 8 bytes of it a tile,
 // 32 lines a load, took as long as the codes (59 us there).  So two tiles' come together, 16
@@ -95,7 +101,8 @@ struct Narrow {
     int pair_in = kAtScales;
     auto load = [&](auto even, int tile, char* slot) __attribute__((always_inline)) {
       const unsigned size = __builtin_amdgcn_readfirstlane(tile < n ? -1 : 0);
-      const int t = p.first + tile;
+      const int turned = ONCE ? tile + p.turn : tile;
+      const int t = p.first + (turned < n ? turned : turned - n);
       if constexpr (decltype(even)::value) {
 #pragma unroll
         for (int i = 0; i < kScaleEach; ++i) {
@@ -237,7 +244,7 @@ DEVINLINE void tile(const MxProduct& p, char* lds) {
                           p.x1 == nullptr ? nullptr : p.x1 + x_base * (p.pitch / 4),
                           p.xs + x_base * xs_pitch, p.w + w_base * (p.K / 2),
                           p.ws + w_base * xs_pitch, p.pitch, p.K / 2, part * p.depth,
-                          tiles_of_k};
+                          tiles_of_k, p.parts == 1 ? n0 / COLS * 2 % tiles_of_k : 0};
   // acc[i][j][r]: row i * 16 + col of x, row j * 16 + quad * 4 + r of the wave's of W
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

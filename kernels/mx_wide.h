@@ -36,6 +36,7 @@ struct Operands {
   int pitch;     // of x and of scales: inputs of a row, whole pairs of tiles
   int k_bytes;   // of a row of W
   int first, tiles;
+  int turn;      // the tile (even) that a loop which may begin anywhere begins with
 };
 
 // One of two places (of values: of an operand's fields the compiler would choose by address, which
