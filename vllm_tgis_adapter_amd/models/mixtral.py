@@ -80,6 +80,18 @@ class MoEBlock(nn.Module):
         h = ops.moe_gemm(x, self.w13, seg, gated=True, rows=rows)
         return ops.moe_gemm(h, self.w2, seg, gated=False)
 
+    def _add_pairs_(self, out, tokens, order, terms) -> None:
+        """Adds the weighted terms of token-expert pairs, listed in `order`, to their tokens.
+        With microscaled weights a token's terms are taken in the order of its choices: atomic
+        sums of more than two may differ from run to run."""
+        if self.mx_act_bits is None:
+            out.index_add_(0, tokens, terms)
+            return
+        pairs = torch.empty_like(terms)
+        pairs[order] = terms
+        for pair in pairs.view(out.shape[0], self.top_k, self.hidden).unbind(1):
+            out += pair
+
     def _forward_ep(self, x: torch.Tensor, flat_ids, flat_w, token_idx):
         """Dispatch token copies to their experts' owner ranks (all-to-all),
         compute locally at full intermediate width, return and combine.
@@ -126,8 +138,8 @@ class MoEBlock(nn.Module):
         y_home = x.new_empty((sum(send_sizes), self.hidden))
         dist.all_to_all_single(y_home, ye.contiguous(), send_sizes, recv_sizes)
         out = torch.zeros_like(x)
-        out.index_add_(0, token_idx[send_order],
-                       y_home * flat_w[send_order, None])
+        self._add_pairs_(out, token_idx[send_order], send_order,
+                         y_home * flat_w[send_order, None])
         return out
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:  # [T, H]
@@ -160,7 +172,7 @@ class MoEBlock(nn.Module):
             seg[1:] = counts.cumsum(0).to(torch.int32)
             xs = x[rows].contiguous()
             ye = self._products(xs, seg)
-            out.index_add_(0, rows, ye * flat_w[sort_idx, None])
+            self._add_pairs_(out, rows, sort_idx, ye * flat_w[sort_idx, None])
             return tp_all_reduce(out)
         # Launch-only expert loop: no data-dependent host branches (`any()`
         # would sync per expert and break hipGraph capture); empty selections
