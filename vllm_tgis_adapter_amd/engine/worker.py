@@ -274,19 +274,28 @@ class Worker:
         )
 
         act_bits = 4 if method == "mxfp4a4" else 6
-        count = 0
-        for mod in self.model.modules():
+        count, left = 0, []
+        for name, mod in self.model.named_modules():
             if isinstance(mod, MoEBlock):
-                count += mod.quantize_mx_(act_bits)
+                made = mod.quantize_mx_(act_bits)
             elif (isinstance(mod, (ColumnParallelLinear, MergedColumnParallelLinear,
                                    RowParallelLinear))
-                  and hasattr(mod, "weight") and mod.weight.shape[1] % 32 == 0):
-                quantize_module_mx_(mod, act_bits)
-                count += 1
+                  and hasattr(mod, "weight")):
+                made = int(mod.weight.shape[1] % 32 == 0)
+                if made:
+                    quantize_module_mx_(mod, act_bits)
+            else:
+                continue
+            count += made
+            if not made:
+                left.append(name)
         if self.device == "cuda":
             torch.cuda.empty_cache()
         print(f"[worker] quantized {count} products' weights to microscaled 4 bits, "
               f"their rows to {act_bits} ({method})", flush=True)
+        if left:
+            print(f"[worker] left {len(left)} as they are, whose inputs (a rank's) are not whole "
+                  f"blocks of 32: {', '.join(left)}", flush=True)
 
     def add_lora(self, lora_path: str, lora_int_id: int) -> None:
         from .lora import load_lora_adapter
