@@ -1,4 +1,4 @@
-"""Which layers microscaled weights leave alone, and that a user is told."""
+"""Which layers microscaled weights leave alone, and that a user is told; calls with nothing in them."""
 
 from types import SimpleNamespace
 
@@ -6,6 +6,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from vllm_tgis_adapter_amd import ops
 from vllm_tgis_adapter_amd.engine.worker import Worker
 from vllm_tgis_adapter_amd.parallel.layers import ColumnParallelLinear, RowParallelLinear
 
@@ -28,3 +29,23 @@ def test_nothing_is_said_where_all_are_rounded(capsys):
     model = nn.ModuleDict({"fits": ColumnParallelLinear(64, 8, dtype=torch.float32)})
     Worker._quantize_model_mx(SimpleNamespace(model=model, device="cpu"), "mxfp4")
     assert "left" not in capsys.readouterr().out
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_single_values_and_rows_without_blocks(device):
+    """The same answers on the CPU and on the GPU."""
+    one = torch.ones((), device=device)
+    byte = torch.ones((), dtype=torch.uint8, device=device)
+    wq, scales = ops.quantize_mx(torch.ones(6, 64, device=device))
+    seg = torch.tensor([0, 1, 1], dtype=torch.int32, device=device)
+    for call in (lambda: ops.quantize_mx(one), lambda: ops.dequantize_mx(wq, byte),
+                 lambda: ops.linear_mx(one, wq, scales), lambda: ops.gated_mx(one, wq, scales),
+                 lambda: ops.moe_gemm_mx(one, wq.view(2, 3, -1), scales.view(2, 3, -1), seg, False)):
+        with pytest.raises(ValueError):
+            call()
+    for bits in (4, 6):
+        y = ops.dequantize_mx(wq[:, :0], scales[:, :0], bits, torch.float16)
+        assert y.shape == (6, 0) and y.dtype == torch.float16

@@ -442,9 +442,14 @@ def _check_mx_bits(bits: int) -> None:
         raise ValueError(f"microscaled codes have 4 or 6 bits, not {bits}")
 
 
-def _check_mx_blocks(k: int) -> None:
+def _check_mx_blocks(x: torch.Tensor) -> int:
+    """Values of a row of x."""
+    if not x.dim():
+        raise ValueError("rows expected, not one value")
+    k = x.shape[-1]
     if k == 0 or k % reference.MX_BLOCK:
         raise ValueError(f"rows of whole blocks of {reference.MX_BLOCK} values expected, not {k}")
+    return k
 
 
 def quantize_mx(x: torch.Tensor, bits: int = 4) -> tuple[torch.Tensor, torch.Tensor]:
@@ -459,10 +464,9 @@ def quantize_mx(x: torch.Tensor, bits: int = 4) -> tuple[torch.Tensor, torch.Ten
     if _native(x):
         return _C.quantize_mx(x, bits)
     _check_mx_bits(bits)
-    _check_mx_blocks(x.shape[-1])
+    lead, k = x.shape[:-1], _check_mx_blocks(x)
     if x.dtype not in _MX_TYPES:
         raise ValueError(f"bfloat16, float16 or float32 expected, not {x.dtype}")
-    lead, k = x.shape[:-1], x.shape[-1]
     codes, scales = reference.quantize_mx(x.detach().reshape(-1, k), bits)
     return (codes.view(*lead, k * bits // 8),
             scales.view(*lead, k // reference.MX_BLOCK))
@@ -479,9 +483,13 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, bits: int = 4,
         raise ValueError("codes and scales of uint8 expected")
     if dtype not in _MX_TYPES:
         raise ValueError(f"bfloat16, float16 or float32 expected, not {dtype}")
+    if not scales.dim():
+        raise ValueError("scales of rows expected, not one value")
     k = scales.shape[-1] * reference.MX_BLOCK
     if codes.shape != (*scales.shape[:-1], k * bits // 8):
         raise ValueError(f"codes {tuple(codes.shape)} do not fit scales {tuple(scales.shape)}")
+    if not codes.numel():
+        return torch.empty((*scales.shape[:-1], k), dtype=dtype, device=codes.device)
     return reference.dequantize_mx(codes.reshape(-1, codes.shape[-1]),
                                    scales.reshape(-1, scales.shape[-1]),
                                    bits).to(dtype).view(*scales.shape[:-1], k)
@@ -491,8 +499,7 @@ def _check_mx_product(x, wq, scales, act_bits: int, halves: int, dims: int, bias
     """Outputs of a product of rows x with microscaled weights, whose arguments it checks
     (the extension checks its own: a small step is bound by the host)."""
     _check_mx_bits(act_bits)
-    k = x.shape[-1]
-    _check_mx_blocks(k)
+    k = _check_mx_blocks(x)
     if x.dtype not in _MX_TYPES:
         raise ValueError(f"bfloat16, float16 or float32 expected, not {x.dtype}")
     if wq.dtype != torch.uint8 or scales.dtype != torch.uint8:
