@@ -5,14 +5,16 @@
 // plain, gated (silu of the first half of W's rows times the second) and over experts'
 // segments (moe_tiles.h).  A lane of v_mfma_scale_f32_16x16x128_f8f6f4 has a row's block of 32
 // values, 16 bytes of 4-bit codes, and its scale, so codes go from memory to LDS to the matrix
-// unit as they are.  6-bit codes of x make exact products as well, at the same rate; 8-bit ones
-// would not: next to 4-bit numbers the unit adds their products up in too few bits
-// (1024 inputs: 4e-6 to 1.3e-5 of the result off, 6 and 4 bits 3e-8).
+// unit as they are.  6-bit codes of x make exact products as well, in as many cycles (with values
+// from registers 6.8 PFLOP/s where 4 bits have 7.3: the clock falls further); 8-bit ones would
+// not: next to 4-bit numbers the unit adds their products up in too few bits (1024 inputs: 4e-6
+// to 1.3e-5 of the result off, 6 and 4 bits 3e-8).
 //
 // Tiles of BM x BN, 256 inputs at a time: rows of 128 bytes, whole cache lines, loaded straight
-// to LDS, and the scales of two such tiles at a time (K is taken in pairs of tiles).  Of a tile's eight blocks a lane of quarter q takes the blocks 2q and 2q + 1 in two
-// products, whose scale bytes are neighbours: one read of two bytes serves both.  Which tile and
-// how many parts of K: mx_plan; few rows have mx_few.hip.
+// to LDS, and the scales of two such tiles at a time (K is taken in pairs of tiles).  Of a tile's
+// eight blocks a lane of quarter q takes the blocks 2q and 2q + 1 in two products, whose scale
+// bytes are neighbours: one read of two bytes serves both.  Which tile and how many parts of K:
+// mx_plan; few rows have mx_few.hip.
 
 #include <algorithm>
 

@@ -4,20 +4,23 @@
 // A tile of 256 inputs is 128 bytes a row, whole cache lines, and what counts is to have
 // enough of them on their way without a pause of the matrix unit:
 //  - Memory comes in slots of half of the rows of x and of W, SLOTS of them in LDS, each
-//    asked for SLOTS - 1 half tiles ahead.  A half tile is half of the rows of x
-//    times all of W, one half after the other; W's halves take turns in order from tile to tile (x0 w0, x1 w1 | x0 w1, x1 w0), so that each quarter of the products
-//    reads one half of an operand into the registers of one that is done with.
+//    asked for SLOTS - 1 half tiles ahead.  A half tile is half of the rows of x times all of
+//    W, one half after the other; W's halves take turns in order from tile to tile (x0 w0,
+//    x1 w1 | x0 w1, x1 w0), so that each quarter of the products reads one half of an operand
+//    into the registers of one that is done with.
 //  - Scales come two tiles' at a time, 16 bytes a row and lane, a round of two tiles ahead (8 bytes
 //    of a tile, two lanes a row, held up the codes: 128 x 128 tiles took 351 us instead of 278 for the
 //    product below, 256 x 256 ones 171 instead of 155 of zeros).
 //  - One barrier a half tile.  Reads and loads stand between the products in source order.
 // The accumulation registers are named in the products themselves (multiply0 below).
 //
-// 8192 rows, 14336 to 4096, 4 bits: 206 us, 4.7 PFLOP/s; whole tiles in two slots by eight waves 290.
-// Bound by the chip's power (a clock of 1.9 GHz; the products alone, from registers, run at 7.3
-// PFLOP/s with such values and 9.7 with zeros): of zeros the loop takes 155 us, without loads 134,
-// without reads of LDS or barriers no less.  Products of 32 x 32 are no faster with zeros and slower by
-// their power (6.5).
+// 8192 rows, 14336 to 4096: 205 us of 4 bits, 4.7 PFLOP/s, and 237 of 6; whole tiles in two slots
+// by eight waves 290.  Bound by stalls first: the matrix unit is busy for 57 % of the cycles (6
+// bits 50 %), with zeros, which the clock does not fall so for, 55 % (177 us); from registers it
+// is for 93 %.  The chip's power is behind the rest: the clock is 1.87 GHz with values and 2.26
+// with zeros (from registers 1.89, 7.3 PFLOP/s, and 2.39, 9.6).  In a program of its own, all of
+// zeros, the loop took 155 us, without loads 134, without reads of LDS or barriers no less.
+// Products of 32 x 32 are no faster with zeros and slower with values (6.5 PFLOP/s).
 #pragma once
 
 #include <type_traits>
