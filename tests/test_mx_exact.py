@@ -154,3 +154,28 @@ def test_form(form, cut, rows, n, k, experts, bits, gated):
     plan = ops._C.mx_plan(rows, n, k, experts, bits, gated)
     assert plan[1:4] == form and (plan[4] > 1) == cut
     check(rows, n, k, experts, bits, gated, "cuda")
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_small_numbers(m, dtype, bits, device):
+    """Rows, terms and results below a type's least normal number: one term a result, and sums
+    of 32 equal ones, are the exact ones rounded once."""
+    g = torch.Generator().manual_seed(m)
+    one, all_ = torch.zeros(8, 64), torch.zeros(8, 64)
+    one[:, :8] = torch.eye(8)
+    all_[:, :32] = 1.0
+    for of_x in (-149, -140, -133, -127, -126, -125, -24, -20, -16):
+        x = (torch.randn(m, 64, generator=g).double() * 2.0 ** of_x).to(dtype)
+        flat = torch.full((m, 64), 2.0 ** of_x, dtype=torch.float64).to(dtype)
+        for of_w in (-20, 0, 20):
+            wq, scales = (t.to(device) for t in ops.quantize_mx(one * 2.0 ** of_w))
+            want = oracle.quantize(x, bits)[2][:, :8] * 2.0 ** of_w
+            got = ops.linear_mx(x.to(device), wq, scales, act_bits=bits).cpu()
+            assert torch.equal(got, want.to(dtype)), (of_x, of_w)
+            wq, scales = (t.to(device) for t in ops.quantize_mx(all_ * 2.0 ** of_w))
+            want = oracle.quantize(flat, bits)[2][:, :8] * 32 * 2.0 ** of_w
+            got = ops.linear_mx(flat.to(device), wq, scales, act_bits=bits).cpu()
+            assert torch.equal(got, want.to(dtype)), (of_x, of_w)

@@ -522,8 +522,8 @@ def linear_mx(x: torch.Tensor, wq: torch.Tensor, scales: torch.Tensor,
               bias: torch.Tensor | None = None, act_bits: int = 4) -> torch.Tensor:
     """Q(x) W^T (+ bias) for 4-bit weights as ``quantize_mx`` makes them (wq [N, K / 2], scales
     [N, K / 32]) and rows x [..., K] that are rounded to `act_bits` the same way inside; sums
-    in 32 bits (what is below 2^-126 may count as zero in them on the GPU), results in x's type.
-    Any N, any number of rows, K a multiple of 32; up to 2^33 weights."""
+    in 32 bits, results in x's type (numbers below its least normal one too).  Any N, any number
+    of rows, K a multiple of 32; up to 2^33 weights."""
     if _native(x):
         return _C.mx_product(x, wq, scales, bias, act_bits)
     n = _check_mx_product(x, wq, scales, act_bits, 1, 2, bias)
